@@ -54,6 +54,10 @@ def _launch(device, name, *args):
             _lib().launch(name, *args, _stream(index))
 
 
+# Kernels write through pointers: raising the version of the tensors that they wrote lets
+# autograd refuse a backward pass that has saved one of them, as for PyTorch's own in-place calls.
+_wrote = torch.autograd.graph.increment_version
+
 _status_words = {}
 
 
@@ -273,6 +277,8 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None, first=None, s
     first [batch]; log_decay, scale and state as there.  The new memory goes to
     `state_out` (dense float32 like state; `state` itself for an update in
     place), or to a new tensor.  Returns (out [batch, heads, dv], new state).
+    An update in place counts as one for autograd: a backward pass that has
+    saved the old memory is refused.
     Acting keeps no graph: arguments that require gradients are refused.
     """
     _require(state is not None, 'decay_attention_step needs a state')
@@ -291,8 +297,11 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None, first=None, s
             apart = abs(state_out.data_ptr() - state.data_ptr())
             _require(apart >= 4 * max(span, state.numel()) or (apart == 0 and dense),
                      'state_out must be state itself or share no memory with it')
-    return _attention_forward(_rows(q), _rows(k), _rows(v), log_decay.contiguous(), state.contiguous(), first, None,
-                              scale, state_out)
+    result = _attention_forward(_rows(q), _rows(k), _rows(v), log_decay.contiguous(), state.contiguous(), first, None,
+                                scale, state_out)
+    if state_out is not None:
+        _wrote(state_out)
+    return result
 
 
 # ---- layer norm ------------------------------------------------------------
@@ -415,7 +424,7 @@ def clip_grad_norm(grads, max_norm, *, eps=1e-6, out=None):
     _require(len(to) == len(grads), 'out has %d tensors for %d gradients', len(to), len(grads))
     max_norm, eps = float(max_norm), float(eps)
     _require(max_norm >= 0 and eps >= 0, 'max_norm and eps must not be negative')
-    table, device = [], None
+    table, written, device = [], [], None
     for g, d in zip(grads, to):
         if g is None:
             _require(d is None, 'out has a tensor where there is no gradient')
@@ -433,6 +442,7 @@ def clip_grad_norm(grads, max_norm, *, eps=1e-6, out=None):
                            or d.stride() != g.stride()):
             raise ValueError('out must match its gradient in shape, type, strides and device')
         table += (g.data_ptr(), d.data_ptr(), g.numel(), DTYPES[dtype])
+        written.append(d)
     if device is None:
         raise ValueError('clip_grad_norm needs at least one gradient')
     _require(device.type == 'cuda', 'clip_grad_norm needs CUDA tensors')
@@ -441,4 +451,5 @@ def clip_grad_norm(grads, max_norm, *, eps=1e-6, out=None):
     norm = torch.empty((), dtype=torch.float32, device=device)
     workspace = torch.empty(_lib().size('clip', table, count), dtype=torch.uint8, device=device)
     _launch(device, 'clip', table, count, max_norm, eps, norm.data_ptr(), workspace.data_ptr())
+    _wrote(written)
     return norm

@@ -1,0 +1,43 @@
+"""What a call of the learned-policy operators leaves behind, and what it must not depend on."""
+import pytest
+
+torch = pytest.importorskip('torch')
+pytestmark = pytest.mark.gpu
+
+from gpu_libero_b200 import policy  # noqa: E402
+from test_gpu_policy import inputs  # noqa: E402
+
+
+# ---- writes that autograd sees -------------------------------------------------
+def test_backward_refuses_a_memory_that_acting_overwrote():
+    t = inputs(2, 5, 2, 2, 8, 8, torch.float32)
+    t['q'].requires_grad_()
+    token = [t[n].detach()[:, 0] for n in 'qkv'] + [t['log_decay']]
+    out, _ = policy.decay_attention(**t)
+    policy.decay_attention_step(*token, t['state'])  # into a new tensor: nothing is overwritten
+    torch.autograd.grad(out.sum(), t['q'], retain_graph=True)
+    policy.decay_attention_step(*token, t['state'], state_out=t['state'])
+    with pytest.raises(RuntimeError, match='inplace operation'):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize('into', [False, True])
+def test_backward_refuses_values_that_clipping_overwrote(into):
+    x, w = torch.randn(9, device='cuda'), torch.ones(9, device='cuda', requires_grad=True)
+    y, z = (x * w).sum(), torch.randn(9, device='cuda')
+    if into:
+        policy.clip_grad_norm([z], 0.1, out=[x])
+    else:
+        policy.clip_grad_norm([x], 0.1)
+    with pytest.raises(RuntimeError, match='inplace operation'):
+        y.backward()
+
+
+def test_writes_to_inference_tensors():
+    with torch.inference_mode():
+        t = inputs(2, 1, 2, 2, 8, 8, torch.float32)
+        token = [t[n][:, 0] for n in 'qkv'] + [t['log_decay']]
+        want = policy.decay_attention_step(*token, t['state'])[1]
+        assert torch.equal(policy.decay_attention_step(*token, t['state'], state_out=t['state'])[1], want)
+        g = torch.full((4,), 2.0, device='cuda')
+        assert float(policy.clip_grad_norm([g], 2.0)) == 4 and bool(((g - 1).abs() < 1e-6).all())
