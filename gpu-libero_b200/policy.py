@@ -22,6 +22,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native
 
@@ -95,6 +96,15 @@ def _ptr(t):
 def _require(condition, message, *values):
     if not condition:
         raise ValueError(message % values if values else message)
+
+
+def _refuse_tangents(*tensors):
+    """Forward-mode derivatives are refused: the kernels would drop them without a word."""
+    if getattr(forward_ad, '_current_level', 0) < 0:  # outside every dual level (a tensor has no tangent there)
+        return
+    for t in tensors:
+        _require(not isinstance(t, torch.Tensor) or forward_ad.unpack_dual(t).tangent is None,
+                 'the policy operators have no forward-mode derivatives')
 
 
 def _rows(t):
@@ -256,9 +266,10 @@ def decay_attention(q, k, v, log_decay, *, scale=None, state=None, first=None, l
 
     Returns (out [batch, time, heads, dv] in q's type, state [batch, heads, dk,
     dv] in float32 after each row's last token).  Differentiable in q, k, v
-    and state, once.  Tokens of a row must be finite; those behind its length
-    may hold anything.
+    and state, once (not in forward mode).  Tokens of a row must be finite;
+    those behind its length may hold anything.
     """
+    _refuse_tangents(q, k, v, log_decay, state)
     scale = _check_attention(q, k, v, log_decay, state, first, lengths, scale, ('batch', 'time'))
     q, k, v = _rows(q), _rows(k), _rows(v)
     log_decay = log_decay.contiguous()
@@ -282,6 +293,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None, first=None, s
     Acting keeps no graph: arguments that require gradients are refused.
     """
     _require(state is not None, 'decay_attention_step needs a state')
+    _refuse_tangents(q, k, v, log_decay, state, state_out)
     scale = _check_attention(q, k, v, log_decay, state, first, None, scale, ('batch',))
     if torch.is_grad_enabled():
         _require(not (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad),
@@ -371,8 +383,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     weight and bias [width]: x's type or float32, both the same, or None.
     Returns a dense tensor of x's shape and type.  Mean, variance and the sums
     of the gradients are held in float32.  Differentiable in x, weight and
-    bias, once; gradients of weight and bias are summed in a fixed order.
+    bias, once (not in forward mode); gradients of weight and bias are summed in
+    a fixed order.
     """
+    _refuse_tangents(x, weight, bias)
     dtype, width, eps = x.dtype, x.shape[-1] if x.dim() else 0, float(eps)
     if not (dtype in DTYPES and width and x.is_cuda and 0 <= eps < math.inf
             and (weight is None or (weight.shape == (width,) and weight.device == x.device
@@ -421,6 +435,7 @@ def clip_grad_norm(grads, max_norm, *, eps=1e-6, out=None):
     """
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     to = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    _refuse_tangents(*grads, *to)
     _require(len(to) == len(grads), 'out has %d tensors for %d gradients', len(to), len(grads))
     max_norm, eps = float(max_norm), float(eps)
     _require(max_norm >= 0 and eps >= 0, 'max_norm and eps must not be negative')

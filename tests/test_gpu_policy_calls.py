@@ -41,3 +41,21 @@ def test_writes_to_inference_tensors():
         assert torch.equal(policy.decay_attention_step(*token, t['state'], state_out=t['state'])[1], want)
         g = torch.full((4,), 2.0, device='cuda')
         assert float(policy.clip_grad_norm([g], 2.0)) == 4 and bool(((g - 1).abs() < 1e-6).all())
+
+
+# ---- forward mode --------------------------------------------------------------
+def test_forward_mode_is_refused_and_plain_tensors_are_not():
+    from torch.autograd import forward_ad
+    t = inputs(2, 5, 2, 2, 8, 8, torch.float32)
+    x = torch.randn((3, 8), device='cuda')
+    want = policy.decay_attention(**t)[0]
+    with forward_ad.dual_level():
+        for n in ('q', 'k', 'v', 'state'):
+            with pytest.raises(ValueError, match='forward-mode'):
+                policy.decay_attention(**dict(t, **{n: forward_ad.make_dual(t[n], torch.ones_like(t[n]))}))
+        with pytest.raises(ValueError, match='forward-mode'):
+            policy.layer_norm(forward_ad.make_dual(x, x))
+        assert torch.equal(policy.decay_attention(**t)[0], want)
+    q = t['q'].clone()
+    with pytest.raises(ValueError, match='forward-mode'):
+        torch.func.jvp(lambda q: policy.decay_attention(**dict(t, q=q))[0], (q,), (q,))
