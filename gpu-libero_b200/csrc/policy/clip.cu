@@ -11,6 +11,8 @@
 // tensors' sizes fix; every CTA of the second pass adds the partial sums itself,
 // which saves a launch between the passes.
 #include <algorithm>
+#include <memory>
+#include <new>
 #include "common.cuh"
 
 namespace {
@@ -160,6 +162,34 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kFew = 96, kMany = 1000;
 static_assert(sizeof(Table<kMany>) < 32000, "kernel arguments");
 
+// Whether memory that is written is also read or written through another entry (0 or
+// 1), or an error: CTAs take the entries in no order, so such a value would be scaled
+// once or twice by chance.
+int shares_memory(const B200ClipTensor *t, int count) {
+  struct Range {
+    uintptr_t low, high;
+    bool write;
+  } few[2 * kFew];
+  std::unique_ptr<Range[]> many(count > kFew ? new (std::nothrow) Range[2 * (size_t)count] : nullptr);
+  Range *ranges = count > kFew ? many.get() : few;
+  if (!ranges) return -(int)cudaErrorMemoryAllocation;
+  size_t n = 0;
+  for (int i = 0; i < count; ++i) {
+    if (!t[i].count) continue;
+    const size_t size = (size_t)t[i].count * element_bytes((int)t[i].dtype);
+    ranges[n++] = {(uintptr_t)t[i].dst, (uintptr_t)t[i].dst + size, true};
+    if (t[i].src != t[i].dst) ranges[n++] = {(uintptr_t)t[i].src, (uintptr_t)t[i].src + size, false};
+  }
+  std::sort(ranges, ranges + n, [](const Range &a, const Range &b) { return a.low < b.low; });
+  uintptr_t written = 0, taken = 0;  // ends of what has been written, and of all
+  for (size_t i = 0; i < n; ++i) {
+    if (ranges[i].low < (ranges[i].write ? taken : written)) return 1;
+    taken = std::max(taken, ranges[i].high);
+    if (ranges[i].write) written = std::max(written, ranges[i].high);
+  }
+  return 0;
+}
+
 int per_launch(int count) { return count <= kFew ? kFew : kMany; }
 int launches(int count) { return std::max(1, (count + per_launch(count) - 1) / per_launch(count)); }
 
@@ -217,6 +247,7 @@ int b200policy_clip(const B200ClipTensor *tensors, int count, float max_norm, fl
   for (int i = 0; i < count; ++i)
     if (tensors[i].count < 0 || tensors[i].dtype < B200_FP32 || tensors[i].dtype > B200_BF16)
       return (int)cudaErrorInvalidValue;
+  if (const int shared = shares_memory(tensors, count)) return shared < 0 ? -shared : (int)cudaErrorInvalidValue;
   return per_launch(count) == kFew ? run<kFew>(tensors, count, max_norm, eps, norm, (double *)workspace, (cudaStream_t)stream)
                                    : run<kMany>(tensors, count, max_norm, eps, norm, (double *)workspace, (cudaStream_t)stream);
 }

@@ -418,6 +418,23 @@ def _dense(t):
     return True
 
 
+def _explain_overlap(entries):
+    """Raise if memory that a clipping call writes belongs to two of its tensors."""
+    ranges = []
+    for src, dst, count, dtype in zip(*[iter(entries)] * 4):
+        size = count * (4 if dtype == DTYPES[torch.float32] else 2)
+        if size:
+            ranges.append((dst, dst + size, True))
+            if src != dst:
+                ranges.append((src, src + size, False))
+    written = taken = 0
+    for low, high, write in sorted(ranges):
+        _require(low >= (taken if write else written), 'gradients (and out) must not share memory: a value would be '
+                 'scaled more than once')
+        taken = max(taken, high)
+        written = max(written, high) if write else written
+
+
 def clip_grad_norm(grads, max_norm, *, eps=1e-6, out=None):
     """Scale gradients so that their global norm is at most `max_norm`.
 
@@ -427,7 +444,9 @@ def clip_grad_norm(grads, max_norm, *, eps=1e-6, out=None):
     grads: CUDA tensors of one device, of any mix of float32, float16 and
     bfloat16 and any shapes whose memory is dense; None is skipped.  They are
     scaled in place, or into the tensors of `out` (None where grads has None;
-    same shapes, types and strides).  Returns the norm before clipping, a
+    same shapes, types and strides).  What is written may not share memory with
+    another tensor of the call: a gradient that is listed twice in place, or an
+    `out` that overlaps a gradient other than its own, is refused.  Returns the norm before clipping, a
     float32 scalar tensor on the device: nothing waits for it.  The sum of the
     squares is held in 64 bits and its order is fixed.  An infinite norm
     scales to zero (infinities to NaN) and a norm that is not a number makes
@@ -460,11 +479,17 @@ def clip_grad_norm(grads, max_norm, *, eps=1e-6, out=None):
         written.append(d)
     if device is None:
         raise ValueError('clip_grad_norm needs at least one gradient')
-    _require(device.type == 'cuda', 'clip_grad_norm needs CUDA tensors')
+    if device.type != 'cuda':
+        _explain_overlap(table)
+        raise ValueError('clip_grad_norm needs CUDA tensors')
     count = len(table) // 4
-    table = struct.pack('=%dq' % len(table), *table)
+    entries, table = table, struct.pack('=%dq' % len(table), *table)
     norm = torch.empty((), dtype=torch.float32, device=device)
     workspace = torch.empty(_lib().size('clip', table, count), dtype=torch.uint8, device=device)
-    _launch(device, 'clip', table, count, max_norm, eps, norm.data_ptr(), workspace.data_ptr())
+    try:
+        _launch(device, 'clip', table, count, max_norm, eps, norm.data_ptr(), workspace.data_ptr())
+    except RuntimeError:
+        _explain_overlap(entries)  # (the library refuses it; sorting here would cost every call)
+        raise
     _wrote(written)
     return norm

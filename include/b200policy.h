@@ -110,7 +110,9 @@ int b200policy_norm_forward(const B200NormArgs *a, void *stream);
 int b200policy_norm_backward(const B200NormArgs *a, void *stream);
 
 /* norm[0] = sqrt(sum over all tensors of |src|^2); every dst = src *
- * min(1, max_norm / (norm[0] + eps)).  `tensors` is a host array. */
+ * min(1, max_norm / (norm[0] + eps)).  `tensors` is a host array; memory that
+ * is written through one entry may not be read or written through another, and
+ * within an entry only dst == src may overlap (rejected otherwise). */
 size_t b200policy_clip_workspace(const B200ClipTensor *tensors, int count);
 int b200policy_clip(const B200ClipTensor *tensors, int count, float max_norm, float eps, float *norm,
                     void *workspace, void *stream);

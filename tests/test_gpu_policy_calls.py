@@ -59,3 +59,22 @@ def test_forward_mode_is_refused_and_plain_tensors_are_not():
     q = t['q'].clone()
     with pytest.raises(ValueError, match='forward-mode'):
         torch.func.jvp(lambda q: policy.decay_attention(**dict(t, q=q))[0], (q,), (q,))
+
+
+# ---- clipping ------------------------------------------------------------------
+def test_clip_refuses_shared_memory_before_it_writes():
+    g = torch.randn(5000, device='cuda')
+    before = g.clone()
+    for grads, out in [([g, g], None), ([g[:3000], g[2999:]], None), ([g[:2000]], [g[1:2001]]),
+                       ([g[:2000], g[2000:4000]], [torch.empty(2000, device='cuda'), g[:2000]])]:
+        with pytest.raises(ValueError, match='share memory'):
+            policy.clip_grad_norm(grads, 0.5, out=out)
+    assert torch.equal(g, before)
+    # neighbours in any order, and one gradient into two places, are taken
+    to = [torch.empty_like(g) for _ in range(2)]
+    norm = policy.clip_grad_norm([g, g], 1.0, out=to)
+    want = before.double() / (2 * before.double().square().sum()).sqrt()
+    assert torch.equal(to[0], to[1]) and float((to[0] - want).abs().max()) < 1e-6 and torch.equal(g, before)
+    assert abs(float(norm) - float((2 * before.double().square().sum()).sqrt())) < 1e-4
+    policy.clip_grad_norm([g[2500:], g[:2500]], 1.0)
+    assert float((g - before.double() / before.double().norm()).abs().max()) < 1e-6

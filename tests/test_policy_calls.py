@@ -31,3 +31,33 @@ def test_forward_mode_derivatives_are_refused():
     for call, args in calls:
         with pytest.raises(ValueError, match='CUDA'):
             call(*args)
+
+
+# ---- memory that clipping writes through one tensor and touches through another -----
+def clipping_that_shares_memory():
+    g, h = torch.ones(64), torch.ones(8, 8)
+    return [('a gradient twice in place', [g, h, g], None),
+            ('overlapping views in place', [g[:40], g[39:]], None),
+            ('one inside the other', [g, g[8:16]], None),
+            ('two gradients into one', [g, h.view(64)], [torch.ones(64)] * 2),
+            ('into its own, shifted', [g[:32]], [g[1:33]]),
+            ("into another's gradient", [g[:32], g[32:]], [torch.ones(32), g[:32]]),
+            ('many tensors', [torch.ones(3) for _ in range(150)] + [g, g[63:]], None)]
+
+
+@pytest.mark.parametrize('name,grads,out', clipping_that_shares_memory())
+def test_clip_refuses_shared_memory(name, grads, out):
+    with pytest.raises(ValueError, match='share memory'):
+        policy.clip_grad_norm(grads, 1.0, out=out)
+    table = b''.join(policy.native.PolicyLibrary.CLIP.pack(a.data_ptr(), b.data_ptr(), a.numel(), 0)
+                     for a, b in zip(grads, out or grads))
+    with pytest.raises(RuntimeError, match='CUDA error 1$'):  # before any launch
+        policy._lib().launch('clip', table, len(grads), 1.0, 0.0, 256, 256, 0)
+
+
+def test_clip_takes_neighbours_and_shared_sources():
+    g = torch.ones(64)
+    for grads, out in [([g[:32], g[32:]], None), ([g[32:], g[:32]], [g[32:], g[:32]]), ([g, g], [torch.ones(64), torch.ones(64)]),
+                       ([g, g[3:9]], [torch.ones(64), torch.ones(6)]), ([g[:0], g, g[5:5]], None), ([g[:32]], [g[32:]])]:
+        with pytest.raises(ValueError, match='CUDA'):
+            policy.clip_grad_norm(grads, 1.0, out=out)
