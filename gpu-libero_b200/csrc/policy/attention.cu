@@ -60,9 +60,12 @@ template <class T, int V> __global__ void __launch_bounds__(kStepThreads) step_k
     v[e] = to_float(((const T *)a.v)[b * a.v_batch + hk * a.v_head + col + e]);
     o[e] = 0.f;
   }
-  // lambda s = s + (lambda - 1) s: lambda itself, rounded, would be off by up to
-  // 2^-25 for a slow decay, and a memory of n tokens by n times that
-  const float forget = expm1f(a.log_decay[h]);
+  // above 1/2, lambda s = s + (lambda - 1) s: lambda itself, rounded, would be off by up
+  // to 2^-25 for a slow decay, and a memory of n tokens by n times that; below, it is
+  // lambda - 1 that loses what is left of s
+  const float lambda = expf(a.log_decay[h]);
+  const bool slow = lambda > 0.5f;
+  const float factor = slow ? expm1f(a.log_decay[h]) : lambda;
   __syncthreads();
   for (int i0 = 0; i0 * rows < dk; i0 += kBatch) {
     if (i0) load(i0);
@@ -73,7 +76,7 @@ template <class T, int V> __global__ void __launch_bounds__(kStepThreads) step_k
       if (live)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          s[i].x[e] = fmaf(s[i].x[e], forget, s[i].x[e]) + k[r] * v[e];
+          s[i].x[e] = fmaf(s[i].x[e], factor, slow ? s[i].x[e] : 0.f) + k[r] * v[e];
           o[e] += q[r] * s[i].x[e];
         }
       *(Block *)(to + r * dv) = s[i];

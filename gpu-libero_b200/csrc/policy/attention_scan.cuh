@@ -442,7 +442,8 @@ template <class T, int KT, int VT, bool TWIN> struct Layout {
   // Two buffers of K and V where four CTAs still fit with them; Q has one, as every
   // warp fetches its own next rows when it has done with the present ones.
   static constexpr int kStages = kState16 && KT <= 64 && !TWIN ? 2 : 1, kStage = kK + kV;
-  // three tables of lambda^m for m of 0 to kTile, each behind 16 zeros
+  // three tables of lambda^m for m of 0 to kTile, each behind 16 zeros (the first
+  // needs none: a whole chunk's decay lies there)
   static constexpr int kTable = 16 + kTile + 1;
   static constexpr int kX = kQ, kTiles = kQ + (TWIN ? kQ : 0) + kStages * kStage;  // X: a twin's queries
   static constexpr int kBytes = kTiles + kS + 3 * kTable * 4 + 2 * 4;
@@ -567,14 +568,16 @@ __global__ void __launch_bounds__(kScanThreads, Layout<T, KT, VT, TWIN>::kReside
   };
   if (chunks) load_queries(0), load_keys(0);
 
-  const float log_decay = p.log_decay[h], whole_left = expf(log_decay * kTile);
+  const float log_decay = p.log_decay[h];
   if (tid < L::kTable) {
     const int m = tid - 16;
     const float x = m > 0 ? expf(log_decay * m) : m == 0 ? 1.f : 0.f;
-    into[m] = x * s.out_scale;
+    if (m >= 0) into[m] = x * s.out_scale;
     within[m] = x * s.pair_scale * s.out_scale;
     kept[m] = x * s.pair_scale;
   }
+  Decay *whole = (Decay *)(into - 16);
+  if (tid == 0) *whole = Decay(log_decay * kTile);
 
   // S: warp owns kM tiles of 16 rows and kN tiles of 8 columns
   constexpr int kM = KT >= 64 ? KT / 64 : 1, kN = KT >= 64 ? VT / 8 : VT / 16;
@@ -794,7 +797,7 @@ __global__ void __launch_bounds__(kScanThreads, Layout<T, KT, VT, TWIN>::kReside
 #pragma unroll
         for (int j = 0; j < kN; ++j) S[i][j][0] = S[i][j][1] = S[i][j][2] = S[i][j][3] = 0.f;
     } else {
-      const float left = rows == kTile ? whole_left : expf(log_decay * rows);
+      const float left = rows == kTile ? whole->at(c) : expf(log_decay * rows);
 #pragma unroll
       for (int i = 0; i < kM; ++i)
 #pragma unroll
@@ -869,7 +872,7 @@ __global__ void __launch_bounds__(kScanThreads, Layout<T, KT, VT, TWIN>::kReside
   }
   if (p.state_only) {
     if (v0 == 0 && tid == 0)
-      p.factors[((int64_t)which * p.batch * p.heads + bh) * p.pieces + piece] = cut ? 0.f : own ? expf(log_decay * own) : 1.f;
+      p.factors[((int64_t)which * p.batch * p.heads + bh) * p.pieces + piece] = cut ? 0.f : own ? Decay(log_decay * own).at(piece) : 1.f;
     return;
   }
   // rows behind the length

@@ -266,7 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
     for (int i = 0; i < 3; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + 8 * i) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const float log_decay = p.log_decay[h], whole_left = expf(log_decay * kRows);
+  const float log_decay = p.log_decay[h];
+  const Decay whole(log_decay * kRows);
   for (int m = tid - 32; m <= kRows; m += kThreads) {
     const float x = m > 0 ? expf(log_decay * m) : m == 0 ? 1.f : 0.f;
     within[m] = x * s.pair_scale * s.out_scale;
@@ -459,10 +460,10 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
     }
 
     // S
+    const float left = rows == kRows ? whole.at(c) : expf(log_decay * rows);
     lost |= !wait(bars + 16, c & 1);
     fence_after();
     {
-      const float left = rows == kRows ? whole_left : expf(log_decay * rows);
 #pragma unroll
       for (int part16 = 0; part16 < 32; part16 += 16) {
         const uint32_t from = mine + kColD + col0 + part16;
@@ -578,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
   }
   if (p.state_only) {
     if (v0 == 0 && tid == 0)
-      p.factors[((int64_t)which * p.batch * p.heads + bh) * p.pieces + piece] = cut ? 0.f : own ? expf(log_decay * own) : 1.f;
+      p.factors[((int64_t)which * p.batch * p.heads + bh) * p.pieces + piece] = cut ? 0.f : own ? Decay(log_decay * own).at(piece) : 1.f;
     return;
   }
   const int end = min(p.piece, p.time - s0);

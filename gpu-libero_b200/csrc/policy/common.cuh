@@ -55,6 +55,23 @@ template <class V> __device__ __forceinline__ V block_sum(V x, V *part) {
   return x;
 }
 
+// What one chunk after another leaves of a memory: w = exp(log_left) each time.  w rounded
+// to 32 bits would be off by the same amount every time (a decay of 1.6e-6 a token by 1.7e-4
+// after 131072 tokens), so the two values around it, 2^-24 apart, take turns as often as
+// w lies near them.  Below 1/2 a memory is gone before that counts.
+struct Decay {
+  float low;
+  uint32_t share;  // of the chunks that take the upper value, times 2^32
+  __device__ __forceinline__ explicit Decay(float log_left) : low(expf(log_left)), share(0) {
+    if (!(low > 0.5f && low <= 1.f)) return;
+    const float rest = (expm1f(log_left) - (low - 1.f)) * 0x1p24f, units = floorf(rest);
+    low += units * 0x1p-24f;
+    share = __float2uint_rz((rest - units) * 0x1p32f);
+  }
+  // the turn comes where the chunks' shares so far pass a whole one
+  __device__ __forceinline__ float at(int chunk) const { return share * (chunk + 1u) < share ? low + 0x1p-24f : low; }
+};
+
 // Two values and the instructions that take both at once.
 struct F2 {
   unsigned long long v;

@@ -78,3 +78,42 @@ def test_clip_refuses_shared_memory_before_it_writes():
     assert abs(float(norm) - float((2 * before.double().square().sum()).sqrt())) < 1e-4
     policy.clip_grad_norm([g[2500:], g[:2500]], 1.0)
     assert float((g - before.double() / before.double().norm()).abs().max()) < 1e-6
+
+
+# ---- decays ---------------------------------------------------------------------
+# With tokens of zero the memory only decays: every chunk of 64 tokens, and every piece
+# of a long row, rounds it once more, independently (the bound that test_gpu_policy.py
+# takes for n roundings of 32 bits).
+@pytest.mark.parametrize('dtype,batch,heads,width,time', [
+    (torch.float32, 5, 32, 8, 1 << 17), (torch.float16, 5, 32, 8, 1 << 17), (torch.bfloat16, 5, 32, 8, 1 << 17),
+    (torch.float32, 1, 1, 8, 1 << 17), (torch.bfloat16, 3, 32, 128, 1 << 16), (torch.bfloat16, 1, 1, 128, 1 << 17)])
+def test_attention_slow_decays_hold_over_long_rows(dtype, batch, heads, width, time):
+    """Whole rows and rows in pieces, on both kernels."""
+    g = torch.Generator('cuda').manual_seed(width)
+    token = torch.zeros((1, 1, 1, width), dtype=dtype, device='cuda').expand(batch, time, heads, width)
+    for i in range(24 // heads + 1):
+        decay = -torch.linspace(1e-6 + i * 3e-8, 2e-6 + i * 3e-8, heads, device='cuda')
+        state = torch.randn((batch, heads, width, width), generator=g, device='cuda')
+        _, last = policy.decay_attention(token, token, token, decay, state=state)
+        want = state.double() * torch.exp(decay.double() * time)[:, None, None]
+        assert bool(((last - want).abs() <= 2.0 ** -24 * (8 + 4 * (time / 64) ** 0.5) * want.abs()).all())
+
+
+@pytest.mark.parametrize('time', [1, 3, 64, 200, 1100])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_attention_decays_of_every_size_keep_what_is_left(dtype, time):
+    """What is left of a memory is right relative to itself, however little that is."""
+    decay = -torch.logspace(-7, 1, 32, device='cuda')
+    for width in (8, 128):
+        token = torch.zeros((2, time, 32, width), dtype=dtype, device='cuda')
+        state = torch.randn((2, 32, width, width), generator=torch.Generator('cuda').manual_seed(1), device='cuda')
+        want = state.double() * torch.exp(decay.double() * time)[:, None, None]
+        last = policy.decay_attention(token, token, token, decay, state=state)[1]
+        steps = state.clone()
+        for t in range(time):
+            policy.decay_attention_step(token[:, t], token[:, t], token[:, t], decay, steps, state_out=steps)
+        for got in (last, steps):
+            kept = want.abs() > 1e-25  # (well above what 32 bits hold)
+            # exp of a rounded product of up to 70 is off by 70 * 2^-24; every step rounds twice
+            bound = 2.0 ** -24 * (80 + 4 * (2 * time) ** 0.5 + 2 * time * (got is steps))
+            assert float(((got - want) / want)[kept].abs().max()) <= bound
