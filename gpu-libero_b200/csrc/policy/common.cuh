@@ -56,8 +56,8 @@ template <class V> __device__ __forceinline__ V block_sum(V x, V *part) {
 }
 
 // What one chunk after another leaves of a memory: w = exp(log_left) each time.  w rounded
-// to 32 bits would be off by the same amount every time (a decay of 1.6e-6 a token by 1.7e-4
-// after 131072 tokens), so the two values around it, 2^-24 apart, take turns as often as
+// to 32 bits would be off by the same amount every time (some decays of 1e-6 to 2e-6 a token by
+// 1.7e-4 after 131072 tokens), so the two values around it, 2^-24 apart, take turns as often as
 // w lies near them.  Below 1/2 a memory is gone before that counts.
 struct Decay {
   float low;

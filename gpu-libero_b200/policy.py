@@ -68,7 +68,8 @@ def _status(device):
     if word is None:
         if device.type != 'cuda' or torch.cuda.is_current_stream_capturing():
             return 0
-        word = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # check() clears it in any mode
+            word = torch.zeros(1, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()  # once: any stream may read it from now on
         _status_words[device] = word
     return word.data_ptr()

@@ -117,3 +117,32 @@ def test_attention_decays_of_every_size_keep_what_is_left(dtype, time):
             # exp of a rounded product of up to 70 is off by 70 * 2^-24; every step rounds twice
             bound = 2.0 ** -24 * (80 + 4 * (2 * time) ** 0.5 + 2 * time * (got is steps))
             assert float(((got - want) / want)[kept].abs().max()) <= bound
+
+
+# ---- the status word --------------------------------------------------------------
+@pytest.fixture
+def no_word():
+    """A process whose status word has not been made yet; the one that was there comes back afterwards."""
+    kept = dict(policy._status_words)
+    policy._status_words.clear()
+    yield
+    torch.cuda.synchronize()
+    policy._status_words.update(kept)
+
+
+def long_wide_row():
+    return inputs(1, 1100, 1, 1, 128, 128, torch.bfloat16)
+
+
+@pytest.mark.parametrize('made,cleared', [(True, False), (False, True), (True, True)])
+def test_check_clears_a_word_of_any_mode(no_word, made, cleared):
+    """Made under inference mode or not, it is cleared under the other."""
+    t = long_wide_row()
+    with torch.inference_mode(made):
+        want = policy.decay_attention(**t)[0].clone()
+    policy._status_words[torch.device('cuda:0')].data.fill_(1)  # raised by hand, as a wait that ran out would
+    with torch.inference_mode(cleared):
+        with pytest.raises(RuntimeError, match='gave up'):
+            policy.check()
+        policy.check()
+    assert torch.equal(policy.decay_attention(**t)[0], want)
