@@ -62,6 +62,7 @@ template <class T> int scan_launch(const ScanParams &p, int kt, int vt, cudaStre
 // bf16 heads wider than 64 on tcgen05 (attention_tc.cu): chunks of 128 tokens,
 // aligned tensors, slices of 64, one CTA an SM.
 constexpr int kTcTile = 128;
-int scan_tc_launch(const ScanParams &p, int *status, cudaStream_t s);
+// call: a number for the status word, not zero, of all launches of one call.
+int scan_tc_launch(const ScanParams &p, int *status, int call, cudaStream_t s);
 
 }  // namespace b200policy

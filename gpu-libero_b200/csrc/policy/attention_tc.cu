@@ -21,8 +21,9 @@
 // for the outputs, 74 us before them for the pieces' states).  Heads of 64 and less
 // keep the warp-level kernel: there a chunk is half the work and the chain as long.
 //
-// Every wait on a barrier is bounded: when one runs out, the CTA sets the status
-// word, and stops after freeing its tensor memory.
+// Every wait on a barrier is bounded: when one runs out, the CTA writes its call's
+// number into the status word, and stops after freeing its tensor memory; the call's
+// other CTAs stop when they see the number, those of other calls do not.
 #include "attention_scan.h"
 #include "common.cuh"
 
@@ -213,7 +214,7 @@ __device__ __noinline__ float state_sum(const bf16 *k, const bf16 *v, int low, i
   return x;
 }
 
-__global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant__ ScanParams p, int *status) {
+__global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant__ ScanParams p, int *status, int call) {
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *W = smem + kW, *Ss = smem + kS;
   float *tables = (float *)(smem + kTables);
@@ -224,8 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
   // a token's row, which is the lane of tensor memory, and the half of its columns
   const int part = warp & 3, half = warp >> 2, token = part * 32 + lane;
 
-  // a wait has run out, here or in another CTA: the outputs are void
-  bool lost = threadIdx.x == 0 && status && *(volatile int *)status;
+  // a wait has run out, here or in another CTA of this call: its outputs are void
+  bool lost = threadIdx.x == 0 && status && *(volatile int *)status == call;
   int unit = blockIdx.x % p.units, which = 0;
   while (unit >= p.scan[which].slices) unit -= p.scan[which++].slices;
   const Scan &s = p.scan[which];
@@ -562,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
   fence_before();
   const bool stop = __syncthreads_or(lost);
   fence_after();
-  if (stop && tid == 0 && status) *status = 1;
+  if (stop && tid == 0 && status) *status = call;
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*(const uint32_t *)(smem + kTmem)), "n"(kColumns));
   if (stop) return;
@@ -593,12 +594,12 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
 }
 }  // namespace tc
 
-int scan_tc_launch(const ScanParams &p, int *status, cudaStream_t stream) {
+int scan_tc_launch(const ScanParams &p, int *status, int call, cudaStream_t stream) {
   const cudaError_t rc = cudaFuncSetAttribute(tc::scan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tc::kBytes);
   if (rc != cudaSuccess) return (int)rc;
   const int64_t grid = (int64_t)p.batch * p.heads * p.pieces * p.units;
   if (grid >= 1ll << 31) return (int)cudaErrorInvalidValue;
-  tc::scan_kernel<<<(unsigned)grid, tc::kThreads, tc::kBytes, stream>>>(p, status);
+  tc::scan_kernel<<<(unsigned)grid, tc::kThreads, tc::kBytes, stream>>>(p, status, call);
   return (int)cudaGetLastError();
 }
 

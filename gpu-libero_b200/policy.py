@@ -76,9 +76,11 @@ def _status(device):
 
 
 def check(device='cuda'):
-    """Raise if a kernel's bounded wait has run out on `device` (the outputs of that call are void).
+    """Raise if a kernel's bounded wait has run out on `device` since the last check.
 
-    Waits for the device; the operators themselves never do."""
+    The outputs of the call that it ran out in are void; which call that was is not known.  Later calls
+    are not affected, except replays of a CUDA graph that holds that call: theirs are void until this
+    check.  Waits for the device; the operators themselves never do."""
     device = torch.device(device)
     if device.index is None:
         device = torch.device(device.type, torch.cuda.current_device())
@@ -87,7 +89,8 @@ def check(device='cuda'):
     if word is not None and int(word.item()):
         word.zero_()
         torch.cuda.synchronize(device)
-        raise RuntimeError('a decay attention kernel gave up waiting on %s; its outputs are void' % device)
+        raise RuntimeError('a decay attention kernel gave up waiting on %s since the last check; the outputs of its call '
+                           'are void' % device)
 
 
 def _ptr(t):

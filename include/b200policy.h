@@ -54,7 +54,8 @@ typedef struct B200AttentionArgs {
   void *dv_out;            /* like v, dense (backward) */
   float *dstate;           /* [batch, heads, dk, dv] or NULL: not wanted (backward) */
   void *workspace;         /* b200policy_attention_workspace() bytes, 16-byte aligned */
-  int32_t *status;         /* set to 1 where a kernel's bounded wait ran out (its outputs are void), or NULL */
+  int32_t *status;         /* or NULL; not zero once a bounded wait of a launch has run out: that launch's outputs
+                            * are void, others are not, but a captured one's replays are until it is set to zero */
   int64_t q_batch, q_time, q_head;
   int64_t k_batch, k_time, k_head;
   int64_t v_batch, v_time, v_head;

@@ -146,3 +146,21 @@ def test_check_clears_a_word_of_any_mode(no_word, made, cleared):
             policy.check()
         policy.check()
     assert torch.equal(policy.decay_attention(**t)[0], want)
+
+
+def test_a_call_does_not_inherit_an_earlier_ones_expired_wait():
+    """The word stays raised for check(), and later calls compute all the same."""
+    t = long_wide_row()
+    leaves = [t[n].requires_grad_() for n in ('q', 'k', 'v', 'state')]
+
+    def both():
+        out, state = policy.decay_attention(**t)
+        return (out, state, *torch.autograd.grad((out, state), leaves, (torch.ones_like(out), torch.ones_like(state))))
+
+    want = both()
+    policy.check()
+    policy._status_words[torch.device('cuda:0')].fill_(1)  # raised by hand, as a wait that ran out would
+    assert all(torch.equal(a, b) for a, b in zip(both(), want))
+    with pytest.raises(RuntimeError, match='gave up'):
+        policy.check()
+    policy.check()
