@@ -247,8 +247,9 @@ Plan plan_of(const B200AttentionArgs *a, bool backward) {
   }
   // Long rows of wide bf16 heads: 16 rows of 2048 tokens and 4 heads of 128 train in
   // 299 us instead of 408, 32 of 1024 in 309 instead of 345; 128 of 256, of which
-  // chunks of 128 leave two, would take 375 instead of 324.
-  r.tc = a->dtype == B200_BF16 && a->time >= 1024 && r.kt > 64;
+  // chunks of 128 leave two, would take 375 instead of 324.  Its waits are bounded:
+  // without a status word, an expired one would pass unseen.
+  r.tc = a->dtype == B200_BF16 && a->time >= 1024 && r.kt > 64 && a->status;
   for (int i = 0; i < p.scans; ++i) {
     const Scan &s = p.scan[i];
     r.tc = r.tc && s.vec_q && s.vec_k && s.vec_v && s.vec_out && s.vd % 8 == 0;

@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
   const int part = warp & 3, half = warp >> 2, token = part * 32 + lane;
 
   // a wait has run out, here or in another CTA of this call: its outputs are void
-  bool lost = threadIdx.x == 0 && status && *(volatile int *)status == call;
+  bool lost = threadIdx.x == 0 && *(volatile int *)status == call;
   int unit = blockIdx.x % p.units, which = 0;
   while (unit >= p.scan[which].slices) unit -= p.scan[which++].slices;
   const Scan &s = p.scan[which];
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
   fence_before();
   const bool stop = __syncthreads_or(lost);
   fence_after();
-  if (stop && tid == 0 && status) *status = call;
+  if (stop && tid == 0) *status = call;
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*(const uint32_t *)(smem + kTmem)), "n"(kColumns));
   if (stop) return;

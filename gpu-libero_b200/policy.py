@@ -63,7 +63,9 @@ _status_words = {}
 
 
 def _status(device):
-    """The address of the device's status word (0 if it would have to be made during a capture)."""
+    """The address of the device's status word.
+
+    Zero if it would have to be made during a capture: such a call takes kernels that need none."""
     word = _status_words.get(device)
     if word is None:
         if device.type != 'cuda' or torch.cuda.is_current_stream_capturing():

@@ -54,8 +54,9 @@ typedef struct B200AttentionArgs {
   void *dv_out;            /* like v, dense (backward) */
   float *dstate;           /* [batch, heads, dk, dv] or NULL: not wanted (backward) */
   void *workspace;         /* b200policy_attention_workspace() bytes, 16-byte aligned */
-  int32_t *status;         /* or NULL; not zero once a bounded wait of a launch has run out: that launch's outputs
-                            * are void, others are not, but a captured one's replays are until it is set to zero */
+  int32_t *status;         /* not zero once a bounded wait of a launch has run out: that launch's outputs are void,
+                            * others are not, but a captured one's replays are until it is set to zero.  NULL: only
+                            * kernels without such waits run (long rows of wide bf16 heads take longer) */
   int64_t q_batch, q_time, q_head;
   int64_t k_batch, k_time, k_head;
   int64_t v_batch, v_time, v_head;

@@ -5,7 +5,7 @@ torch = pytest.importorskip('torch')
 pytestmark = pytest.mark.gpu
 
 from gpu_libero_b200 import policy  # noqa: E402
-from test_gpu_policy import inputs  # noqa: E402
+from test_gpu_policy import close, close_rows, inputs, recurrence  # noqa: E402
 
 
 # ---- writes that autograd sees -------------------------------------------------
@@ -164,3 +164,16 @@ def test_a_call_does_not_inherit_an_earlier_ones_expired_wait():
     with pytest.raises(RuntimeError, match='gave up'):
         policy.check()
     policy.check()
+
+
+def test_a_capture_without_a_status_word(no_word):
+    """A process whose first call is captured: the captured kernels have nothing to report, and are right."""
+    t = long_wide_row()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, state = policy.decay_attention(**t)
+    assert not policy._status_words
+    graph.replay()
+    want, want_state = recurrence(**t)
+    close_rows(out, want, 1228, 'out')
+    close(state, want_state, 1101, 'state')

@@ -61,3 +61,25 @@ def test_clip_takes_neighbours_and_shared_sources():
                        ([g, g[3:9]], [torch.ones(64), torch.ones(6)]), ([g[:0], g, g[5:5]], None), ([g[:32]], [g[32:]])]:
         with pytest.raises(ValueError, match='CUDA'):
             policy.clip_grad_norm(grads, 1.0, out=out)
+
+
+# ---- what the library plans ---------------------------------------------------------
+def attention_workspace(time, heads, dk, dv, dtype=2, batch=1, kv_heads=None, backward=0, status=0):
+    """Bytes that the library asks for a forward or backward pass over dense, aligned tensors."""
+    kv_heads = kv_heads or heads
+    rows = lambda heads, width: (time * heads * width, heads * width, width)  # noqa: E731
+    args = policy.native.PolicyLibrary.ATTENTION.pack(
+        *[256] * 4, 0, 0, 0, *[256] * 8, 0, status, *rows(heads, dk), *rows(kv_heads, dk), *rows(kv_heads, dv),
+        *rows(heads, dv), 0, 0, batch, time, heads, kv_heads, dk, dv, dtype, 1.0)
+    return policy._lib().size('attention', args, backward)
+
+
+def test_bounded_waits_need_a_status_word():
+    """The kernel with bounded waits splits a long row into pieces of one CTA an SM, the other one of several:
+    without a word to report to, the other one runs."""
+    with_word, without = (attention_workspace(8192, 8, 128, 128, status=s) for s in (256, 0))
+    assert with_word and without > 1.5 * with_word
+    # where no kernel has such waits, the word changes nothing
+    for over in (dict(dtype=1), dict(dk=64, dv=64), dict(time=1000)):
+        shape = dict(dict(time=8192, heads=8, dk=128, dv=128), **over)
+        assert attention_workspace(**shape, status=256) == attention_workspace(**shape)
