@@ -293,7 +293,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None, first=None, s
     q [batch, heads, dk], k [batch, kv_heads, dk], v [batch, kv_heads, dv],
     first [batch]; log_decay, scale and state as there.  The new memory goes to
     `state_out` (dense float32 like state; `state` itself for an update in
-    place), or to a new tensor.  Returns (out [batch, heads, dv], new state).
+    place; it may share memory with no other argument), or to a new tensor.  Returns (out [batch, heads, dv], new state).
     An update in place counts as one for autograd: a backward pass that has
     saved the old memory is refused.
     Acting keeps no graph: arguments that require gradients are refused.
@@ -309,12 +309,9 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None, first=None, s
                  and state_out.device == q.device, 'state_out must be dense float32 of shape %s on %s',
                  tuple(state.shape), q.device)
         _require(not (state_out.requires_grad and torch.is_grad_enabled()), 'state_out must not require gradients')
-        if state_out is not state and state.numel():
-            dense = state.is_contiguous()
-            span = state.numel() if dense else 1 + sum((n - 1) * s for n, s in zip(state.shape, state.stride()))
+        if state_out is not state and state.is_contiguous():  # (one that is not is read from a dense copy)
             apart = abs(state_out.data_ptr() - state.data_ptr())
-            _require(apart >= 4 * max(span, state.numel()) or (apart == 0 and dense),
-                     'state_out must be state itself or share no memory with it')
+            _require(apart == 0 or apart >= 4 * state.numel(), 'state_out must be state itself or share no memory with it')
     result = _attention_forward(_rows(q), _rows(k), _rows(v), log_decay.contiguous(), state.contiguous(), first, None,
                                 scale, state_out)
     if state_out is not None:

@@ -177,3 +177,16 @@ def test_a_capture_without_a_status_word(no_word):
     want, want_state = recurrence(**t)
     close_rows(out, want, 1228, 'out')
     close(state, want_state, 1101, 'state')
+
+
+# ---- memories ----------------------------------------------------------------------
+def test_step_takes_a_strided_memory_next_to_its_output():
+    t = inputs(2, 1, 2, 2, 8, 8, torch.float32)
+    token = [t[n][:, 0] for n in 'qkv'] + [t['log_decay']]
+    want = policy.decay_attention_step(*token, t['state'])
+    store = torch.zeros(3 * 256, device='cuda')
+    to, state = store[:256].view(2, 2, 8, 8), store[256:].view(2, 2, 8, 16)[..., :8]
+    state.copy_(t['state'])
+    got = policy.decay_attention_step(*token, state, state_out=to)
+    assert got[1] is to and torch.equal(got[0], want[0]) and torch.equal(to, want[1])
+    assert torch.equal(state, t['state'])
