@@ -421,6 +421,11 @@ def _dense(t):
     return True
 
 
+def _same_order(a, b):
+    """Whether two tensors of one shape lay their elements out alike (strides of single elements do not count)."""
+    return not a.numel() or all(n == 1 or i == j for n, i, j in zip(a.shape, a.stride(), b.stride()))
+
+
 def _explain_overlap(entries):
     """Raise if memory that a clipping call writes belongs to two of its tensors."""
     ranges = []
@@ -476,7 +481,7 @@ def clip_grad_norm(grads, max_norm, *, eps=1e-6, out=None):
             raise ValueError('gradients must fill their memory densely: shape %s, strides %s'
                              % (tuple(g.shape), g.stride()))
         if d is not g and (d is None or d.shape != g.shape or d.dtype is not dtype or d.device != device
-                           or d.stride() != g.stride()):
+                           or (d.stride() != g.stride() and not _same_order(g, d))):
             raise ValueError('out must match its gradient in shape, type, strides and device')
         table += (g.data_ptr(), d.data_ptr(), g.numel(), DTYPES[dtype])
         written.append(d)

@@ -83,3 +83,16 @@ def test_bounded_waits_need_a_status_word():
     for over in (dict(dtype=1), dict(dk=64, dv=64), dict(time=1000)):
         shape = dict(dict(time=8192, heads=8, dk=128, dv=128), **over)
         assert attention_workspace(**shape, status=256) == attention_workspace(**shape)
+
+
+def test_clip_takes_layouts_that_differ_by_single_elements_only():
+    """A 1 x 1 convolution's gradient: the dense order and the channels-last one are the same memory."""
+    g = torch.ones(4, 6, 1, 1)
+    alike = torch.empty(4, 6, 1, 1).to(memory_format=torch.channels_last).as_strided((4, 6, 1, 1), (6, 1, 6, 6))
+    assert g.stride() != alike.stride()
+    for grads, out in (([g], [alike]), ([alike], [g]), ([torch.ones(1, 5)], [torch.ones(5, 1).t()]),
+                       ([torch.ones(2, 0, 5)], [torch.ones(0, 2, 5).transpose(0, 1)])):
+        with pytest.raises(ValueError, match='CUDA'):
+            policy.clip_grad_norm(grads, 1.0, out=out)
+    with pytest.raises(ValueError, match='out must match'):
+        policy.clip_grad_norm([torch.ones(4, 6)], 1.0, out=[torch.ones(6, 4).t()])
