@@ -241,6 +241,7 @@ Plan plan_of(const B200AttentionArgs *a, bool backward) {
   const bool thin = r.kt > 64 && (a->dtype == B200_FP32 || widest <= 96);
   r.vt = widest <= 32 || thin ? 32 : 64;
   for (int i = 0; i < p.scans; ++i) {
+    p.scan[i].vec_final = (uintptr_t)p.scan[i].final % 16 == 0;
     p.scan[i].slices = (p.scan[i].vd + r.vt - 1) / r.vt;
     p.units += p.scan[i].slices;
     p.scan[i].parts = p.scan[i].final ? 3 : 2;
@@ -252,7 +253,7 @@ Plan plan_of(const B200AttentionArgs *a, bool backward) {
   r.tc = a->dtype == B200_BF16 && a->time >= 1024 && r.kt > 64 && a->status;
   for (int i = 0; i < p.scans; ++i) {
     const Scan &s = p.scan[i];
-    r.tc = r.tc && s.vec_q && s.vec_k && s.vec_v && s.vec_out && s.vd % 8 == 0;
+    r.tc = r.tc && s.vec_q && s.vec_k && s.vec_v && s.vec_out && s.vec_final && s.vd % 8 == 0;
   }
   if (r.tc) {
     r.vt = 64;
@@ -318,6 +319,12 @@ bool args_ok(const B200AttentionArgs *a) {
          a->heads % a->kv_heads == 0 && a->dk > 0 && a->dv > 0 && a->dk <= B200_HEAD_MAX && a->dv <= B200_HEAD_MAX &&
          (int64_t)a->batch * a->heads < (1ll << 31);
 }
+// What a launch reads and writes is there (with elements to it: batch is not zero).
+bool pointers_ok(const B200AttentionArgs *a, bool backward) {
+  const bool tokens = !a->time || (a->q && a->k && a->v && (backward ? a->dout && a->dq && a->dk_out && a->dv_out : a->out != nullptr));
+  return tokens && a->log_decay && (backward || a->state_out);
+}
+bool workspace_ok(const Plan &r, const void *workspace) { return !r.bytes() || (workspace && (uintptr_t)workspace % 16 == 0); }
 }  // namespace
 
 extern "C" {
@@ -330,10 +337,12 @@ size_t b200policy_attention_workspace(const B200AttentionArgs *a, int backward) 
 int b200policy_attention_forward(const B200AttentionArgs *a, void *stream) {
   if (!args_ok(a)) return (int)cudaErrorInvalidValue;
   if (a->batch == 0) return 0;
+  if (!pointers_ok(a, false)) return (int)cudaErrorInvalidValue;
   return by_dtype(a->dtype, [&](auto type) {
     using T = decltype(type);
     if (a->time != 1) {
       Plan r = plan_of(a, false);
+      if (!workspace_ok(r, a->workspace)) return (int)cudaErrorInvalidValue;
       return run<T>(r, a->status, (cudaStream_t)stream);
     }
     const unsigned grid = (unsigned)(a->batch * a->heads);
@@ -347,9 +356,11 @@ int b200policy_attention_forward(const B200AttentionArgs *a, void *stream) {
 int b200policy_attention_backward(const B200AttentionArgs *a, void *stream) {
   if (!args_ok(a)) return (int)cudaErrorInvalidValue;
   if (a->batch == 0) return 0;
+  if (!pointers_ok(a, true)) return (int)cudaErrorInvalidValue;
   return by_dtype(a->dtype, [&](auto type) {
     using T = decltype(type);
     Plan r = plan_of(a, true);
+    if (!workspace_ok(r, a->workspace)) return (int)cudaErrorInvalidValue;
     const int rc = run<T>(r, a->status, (cudaStream_t)stream);
     const int64_t tokens = (int64_t)a->batch * a->time;
     if (rc || !r.float_rows || !tokens) return rc;

@@ -853,7 +853,7 @@ __global__ void __launch_bounds__(kScanThreads, Layout<T, KT, VT, TWIN>::kReside
                              : s.final + (int64_t)bh * kd * s.vd;
     const int top = m0 + g, left = n0 + 2 * t;
     to += top * s.vd + v0 + left;
-    const bool pairs = VEC || s.vd % 2 == 0;  // and v0, left are even: 8-byte aligned
+    const bool pairs = VEC || (s.vd % 2 == 0 && (p.state_only || s.vec_final));  // (v0, left are even)
 #pragma unroll
     for (int i = 0; i < kM; ++i)
 #pragma unroll
@@ -915,7 +915,7 @@ template <class T, int KT, int VT, int PARTS> int launch(const ScanParams &p, cu
   for (int i = 0; i < p.scans; ++i) {
     const Scan &s = p.scan[i];
     twin = twin || s.twin_out;
-    vec = vec && s.vec_q && s.vec_k && s.vec_v && s.vec_out && s.vd % 2 == 0 && (!s.twin_out || (s.vec_x && s.vec_twin));
+    vec = vec && s.vec_q && s.vec_k && s.vec_v && s.vec_out && s.vec_final && s.vd % 2 == 0 && (!s.twin_out || (s.vec_x && s.vec_twin));
     full = full && s.kd == KT && s.vd % VT == 0 && !s.out_float && (!s.twin_out || s.vd == VT);
   }
   const int mode = !vec ? 0 : full ? 2 : 1;

@@ -24,7 +24,7 @@ struct Scan {
   int reverse;
   int parts; // terms of the weighted keys in bf16: 3 where `final` is wanted
   float pair_scale, out_scale;
-  int vec_q, vec_k, vec_v, vec_out;  // 16-byte accesses are aligned
+  int vec_q, vec_k, vec_v, vec_out, vec_final;  // 16-byte accesses are aligned
   // A second output with the same state, read the other way round (S transposed):
   //   twin_out_i = sum_{j <= i} w_ij pair_scale (x_i . v_j) k_j + into_i x_i S^T
   // dk beside dv: one state is kept instead of two.  Heads of up to 64, 16-bit.

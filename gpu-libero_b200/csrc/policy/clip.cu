@@ -245,7 +245,8 @@ int b200policy_clip(const B200ClipTensor *tensors, int count, float max_norm, fl
                     void *stream) {
   if (count < 0 || (count && !tensors) || !norm || !workspace) return (int)cudaErrorInvalidValue;
   for (int i = 0; i < count; ++i)
-    if (tensors[i].count < 0 || tensors[i].dtype < B200_FP32 || tensors[i].dtype > B200_BF16)
+    if (tensors[i].count < 0 || tensors[i].dtype < B200_FP32 || tensors[i].dtype > B200_BF16 ||
+        (tensors[i].count && !(tensors[i].src && tensors[i].dst)))
       return (int)cudaErrorInvalidValue;
   if (const int shared = shares_memory(tensors, count)) return shared < 0 ? -shared : (int)cudaErrorInvalidValue;
   return per_launch(count) == kFew ? run<kFew>(tensors, count, max_norm, eps, norm, (double *)workspace, (cudaStream_t)stream)

@@ -622,7 +622,7 @@ template <class W> __global__ void __launch_bounds__(1024) totals_kernel(B200Nor
 
 bool args_ok(const B200NormArgs *a) {
   return a && dtype_ok(a->dtype) && (a->weight_dtype == a->dtype || a->weight_dtype == B200_FP32) && a->rows >= 0 &&
-         a->rows < (1ll << 31) && a->width > 0;
+         a->rows < (1ll << 31) && a->width > 0 && (uintptr_t)a->stats % 8 == 0;
 }
 
 // Calls f with values of the row's and the weight's element types.
@@ -706,6 +706,7 @@ size_t b200policy_norm_workspace(const B200NormArgs *a) {
 int b200policy_norm_forward(const B200NormArgs *a, void *stream) {
   if (!args_ok(a)) return (int)cudaErrorInvalidValue;
   if (a->rows == 0) return 0;
+  if (!a->x || !a->y) return (int)cudaErrorInvalidValue;
   const Plan p = plan_of(a, false);
   return by_types(a, [&](auto type, auto weight) {
     using T = decltype(type);
@@ -729,7 +730,8 @@ int b200policy_norm_forward(const B200NormArgs *a, void *stream) {
 }
 
 int b200policy_norm_backward(const B200NormArgs *a, void *stream) {
-  if (!args_ok(a)) return (int)cudaErrorInvalidValue;
+  if (!args_ok(a) || (a->rows && !(a->x && a->dy && a->stats))) return (int)cudaErrorInvalidValue;
+  if (b200policy_norm_workspace(a) && (!a->workspace || (uintptr_t)a->workspace % 16)) return (int)cudaErrorInvalidValue;
   const Plan p = plan_of(a, true);
   return by_types(a, [&](auto type, auto weight) {
     using T = decltype(type);

@@ -10,7 +10,9 @@
  *   - launch functions return a cudaError_t value (0 == success) and
  *     cudaErrorInvalidValue (1) for rejected arguments;
  *   - every *_bytes() export is checked by the host against its own layout;
- *   - strides are in elements; the innermost dimension is contiguous.
+ *   - strides are in elements; the innermost dimension is contiguous;
+ *   - pointers are aligned to their elements, those marked so to more; what is
+ *     not marked "or NULL" has to be there unless it holds no element.
  */
 #ifndef B200POLICY_H
 #define B200POLICY_H
@@ -74,7 +76,8 @@ typedef struct B200NormArgs {
   const void *weight; /* [width] or NULL: one */
   const void *bias;   /* [width] or NULL: zero */
   void *y;            /* [rows, width], dense (forward) */
-  float *stats;       /* [rows, 2]: mean, rstd (forward writes, backward reads; forward: NULL if not wanted) */
+  float *stats;       /* [rows, 2]: mean, rstd, 8-byte aligned (forward writes, backward reads; forward: NULL if not
+                       * wanted) */
   const void *dy;     /* [rows, width], row stride dy_row (backward) */
   void *dx;           /* [rows, width], dense, or NULL (backward) */
   void *dweight;      /* [width], weight's type, or NULL (backward) */

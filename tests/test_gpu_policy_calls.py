@@ -190,3 +190,21 @@ def test_step_takes_a_strided_memory_next_to_its_output():
     got = policy.decay_attention_step(*token, state, state_out=to)
     assert got[1] is to and torch.equal(got[0], want[0]) and torch.equal(to, want[1])
     assert torch.equal(state, t['state'])
+
+
+@pytest.mark.parametrize('dtype,time,width', [(torch.float32, 70, 8), (torch.float16, 70, 64), (torch.bfloat16, 70, 64),
+                                              (torch.bfloat16, 1100, 128), (torch.float32, 70, 7), (torch.float32, 1, 8)])
+def test_the_library_writes_memories_of_any_alignment(dtype, time, width):
+    """A caller of the C ABI may put the final memory, or its gradient, at any float."""
+    t = inputs(2, time, 2, 2, width, width, dtype)
+    want = policy.decay_attention(**t)
+    store = torch.zeros(2 * 2 * width * width + 3, device='cuda')
+    for shift in (0, 1, 2, 3):
+        to = store[shift:shift + 4 * width * width].view(2, 2, width, width)
+        out, _ = policy._attention_forward(*(t[n] for n in ('q', 'k', 'v', 'log_decay', 'state', 'first', 'lengths', 'scale')),
+                                           state_out=to)
+        # (another alignment may take another kernel)
+        close_rows(out, want[0].double(), time + width)
+        close_rows(to, want[1].double(), time + 1)
+        assert bool((store[:shift] == 0).all()) and bool((store[shift + 4 * width * width:] == 0).all())
+        store.zero_()

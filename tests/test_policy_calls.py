@@ -96,3 +96,47 @@ def test_clip_takes_layouts_that_differ_by_single_elements_only():
             policy.clip_grad_norm(grads, 1.0, out=out)
     with pytest.raises(ValueError, match='out must match'):
         policy.clip_grad_norm([torch.ones(4, 6)], 1.0, out=[torch.ones(6, 4).t()])
+
+
+# ---- sizes and pointers ----------------------------------------------------------
+ATTENTION = ('q k v log_decay state first lengths out state_out dout dstate_out dq dk_out dv_out dstate workspace status '
+             'strides batch time heads kv_heads dk dv dtype scale').split()
+
+
+def attention_args(**over):
+    """A B200AttentionArgs of five tokens whose pointers are all there (and none of which may ever be launched)."""
+    fields = dict.fromkeys(ATTENTION[:17], 4096)
+    fields.update(strides=(80, 16, 8) * 4 + (5, 1), batch=1, time=5, heads=2, kv_heads=1, dk=8, dv=8, dtype=2, scale=1.0)
+    fields.update(over)
+    flat = [x for n in ATTENTION for x in (fields[n] if n == 'strides' else (fields[n],))]
+    return policy.native.PolicyLibrary.ATTENTION.pack(*flat)
+
+
+def norm_args(**over):
+    fields = dict.fromkeys('x weight bias y stats dy dx dweight dbias workspace'.split(), 4096)
+    fields.update(rows=1000, x_row=96, dy_row=96, width=96, dtype=2, weight_dtype=0, eps=1e-5)
+    fields.update(over)
+    return policy.native.PolicyLibrary.NORM.pack(*fields.values())
+
+
+@pytest.mark.parametrize('name,args', [
+    *[('attention_forward', dict([(n, 0)])) for n in ('q', 'k', 'v', 'log_decay', 'out', 'state_out')],
+    *[('attention_forward', dict([(n, 0), ('time', 1)])) for n in ('q', 'out', 'state_out')],
+    *[('attention_backward', dict([(n, 0)])) for n in ('q', 'k', 'v', 'log_decay', 'dout', 'dq', 'dk_out', 'dv_out',
+                                                       'workspace')],
+    ('attention_backward', dict(workspace=4104)),
+    ('attention_forward', dict(time=4096, heads=1, workspace=0)),
+    ('attention_forward', dict(time=4096, heads=1, workspace=4104)),
+    *[('norm_forward', dict([(n, 0)])) for n in ('x', 'y')], ('norm_forward', dict(stats=4100)),
+    *[('norm_backward', dict([(n, 0)])) for n in ('x', 'dy', 'stats', 'workspace')],
+    ('norm_backward', dict(stats=4100)), ('norm_backward', dict(workspace=4104))])
+def test_launches_reject_what_is_not_there_or_not_aligned(name, args):
+    layout = attention_args if name.startswith('attention') else norm_args
+    with pytest.raises(RuntimeError, match='CUDA error 1$'):  # before any launch
+        policy._lib().launch(name, layout(**args), 0)
+
+
+def test_clip_rejects_missing_memory():
+    for src, dst in ((0, 4096), (4096, 0)):
+        with pytest.raises(RuntimeError, match='CUDA error 1$'):
+            policy._lib().launch('clip', policy.native.PolicyLibrary.CLIP.pack(src, dst, 4, 0), 1, 1.0, 0.0, 256, 256, 0)
