@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(256) share_kernel(const float *part_k, const f
 }
 
 constexpr int kSms = 148;
+constexpr int kMostTokens = 0x7fffffff - 1024;  // of a row: token numbers a few chunks on are 32-bit too
 
 bool aligned(const void *p, int64_t batch, int64_t time, int64_t head, int width, size_t bytes) {
   const int64_t block = 16 / (int64_t)bytes;
@@ -271,7 +272,7 @@ Plan plan_of(const B200AttentionArgs *a, bool backward) {
   int64_t pieces = rows && rows < kSms ? std::min<int64_t>((int64_t)resident * kSms / rows, chunks / 2) : 1;
   if (pieces < 2) pieces = 1;
   p.piece = pieces > 1 ? (int)((chunks + pieces - 1) / pieces) * tile : std::max(p.time, 1);
-  p.pieces = pieces > 1 ? (p.time + p.piece - 1) / p.piece : 1;
+  p.pieces = pieces > 1 ? (int)(((int64_t)p.time + p.piece - 1) / p.piece) : 1;
   for (int i = 0; i < p.scans; ++i) {
     p.states_at[i] = (int64_t)r.state_floats;
     r.state_floats += (size_t)p.batch * p.heads * p.pieces * p.scan[i].kd * p.scan[i].vd;
@@ -315,7 +316,7 @@ template <class T> int run(Plan &r, int *status, cudaStream_t stream) {
 }
 
 bool args_ok(const B200AttentionArgs *a) {
-  return a && dtype_ok(a->dtype) && a->batch >= 0 && a->time >= 0 && a->heads > 0 && a->kv_heads > 0 &&
+  return a && dtype_ok(a->dtype) && a->batch >= 0 && a->time >= 0 && a->time <= kMostTokens && a->heads > 0 && a->kv_heads > 0 &&
          a->heads % a->kv_heads == 0 && a->dk > 0 && a->dv > 0 && a->dk <= B200_HEAD_MAX && a->dv <= B200_HEAD_MAX &&
          (int64_t)a->batch * a->heads < (1ll << 31);
 }

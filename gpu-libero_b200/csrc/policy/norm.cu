@@ -23,6 +23,7 @@ using namespace b200policy;
 
 constexpr int kSms = 148;
 constexpr int kWideThreads = 256;
+constexpr int kMostColumns = 0x7fffffff - 1024;  // column numbers a CTA's stride on are 32-bit too
 
 template <class W> __device__ __forceinline__ float weight_at(const void *w, int i, float none) {
   return w ? to_float(((const W *)w)[i]) : none;
@@ -622,7 +623,7 @@ template <class W> __global__ void __launch_bounds__(1024) totals_kernel(B200Nor
 
 bool args_ok(const B200NormArgs *a) {
   return a && dtype_ok(a->dtype) && (a->weight_dtype == a->dtype || a->weight_dtype == B200_FP32) && a->rows >= 0 &&
-         a->rows < (1ll << 31) && a->width > 0 && (uintptr_t)a->stats % 8 == 0;
+         a->rows < (1ll << 31) && a->width > 0 && a->width <= kMostColumns && (uintptr_t)a->stats % 8 == 0;
 }
 
 // Calls f with values of the row's and the weight's element types.

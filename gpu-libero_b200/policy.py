@@ -28,6 +28,7 @@ from . import native
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 HEAD_MAX = 128  # B200_HEAD_MAX of include/b200policy.h
+INDEX_MAX = (1 << 31) - 1 - 1024  # tokens of a row, and columns of a norm: the kernels count them in 32 bits
 ATTENTION_WORKSPACE, NORM_WORKSPACE = 15 * 8, 9 * 8  # offsets of the structs' workspace fields
 
 _library = None
@@ -159,6 +160,7 @@ def _explain_attention(q, k, v, log_decay, state, first, lengths, lead):
     _require(lengths is None or (lengths.shape == at[:1] and lengths.dtype == torch.int32),
              'lengths must be int32 of shape (%d,)', at[0])
     _require(at[0] * heads < 1 << 31, 'too many rows: %d', at[0] * heads)
+    _require(len(at) == 1 or at[1] <= INDEX_MAX, 'too many tokens: %d', at[-1])
     _require(q.is_cuda, 'decay attention needs CUDA tensors')
 
 
@@ -173,6 +175,7 @@ def _check_attention(q, k, v, log_decay, state, first, lengths, scale, lead):
                 and k.device == device and v.device == device and log_decay.device == device
                 and log_decay.dtype is torch.float32 and log_decay.shape == (heads,)
                 and not (log_decay.requires_grad and torch.is_grad_enabled()) and at[0] * heads < 1 << 31
+                and (len(at) == 1 or at[1] <= INDEX_MAX)
                 and (state is None or (state.shape == (at[0], heads, dk, dv) and state.dtype is torch.float32
                                        and state.device == device))
                 and (first is None or (first.shape == at and first.dtype is torch.bool and first.device == device))
@@ -376,6 +379,7 @@ def _explain_norm(x, weight, bias, eps):
     _require(weight is None or bias is None or weight.dtype == bias.dtype, 'weight and bias must have one type')
     _require(eps >= 0 and math.isfinite(eps), 'eps must be finite and not negative')
     _require(x.numel() // x.shape[-1] < 1 << 31, 'too many rows')
+    _require(x.shape[-1] <= INDEX_MAX, 'too many columns: %d', x.shape[-1])
     _require(x.is_cuda, 'layer_norm needs a CUDA tensor')
 
 
@@ -391,7 +395,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """
     _refuse_tangents(x, weight, bias)
     dtype, width, eps = x.dtype, x.shape[-1] if x.dim() else 0, float(eps)
-    if not (dtype in DTYPES and width and x.is_cuda and 0 <= eps < math.inf
+    if not (dtype in DTYPES and 0 < width <= INDEX_MAX and x.is_cuda and 0 <= eps < math.inf
             and (weight is None or (weight.shape == (width,) and weight.device == x.device
                                     and (weight.dtype is dtype or weight.dtype is torch.float32)))
             and (bias is None or (bias.shape == (width,) and bias.device == x.device

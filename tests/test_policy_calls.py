@@ -99,6 +99,16 @@ def test_clip_takes_layouts_that_differ_by_single_elements_only():
 
 
 # ---- sizes and pointers ----------------------------------------------------------
+def test_rows_too_long_to_count_are_refused():
+    many = (1 << 31) - 512
+    q = torch.zeros(1, 1, 1, 8).expand(1, many, 1, 8)
+    with pytest.raises(ValueError, match='too many tokens'):
+        policy.decay_attention(q, q, q, torch.zeros(1))
+    for width in (many, 1 << 31):
+        with pytest.raises(ValueError, match='too many columns'):
+            policy.layer_norm(torch.zeros(2, 1).expand(2, width))
+
+
 ATTENTION = ('q k v log_decay state first lengths out state_out dout dstate_out dq dk_out dv_out dstate workspace status '
              'strides batch time heads kv_heads dk dv dtype scale').split()
 
@@ -124,10 +134,11 @@ def norm_args(**over):
     *[('attention_forward', dict([(n, 0), ('time', 1)])) for n in ('q', 'out', 'state_out')],
     *[('attention_backward', dict([(n, 0)])) for n in ('q', 'k', 'v', 'log_decay', 'dout', 'dq', 'dk_out', 'dv_out',
                                                        'workspace')],
-    ('attention_backward', dict(workspace=4104)),
+    ('attention_backward', dict(workspace=4104)), ('attention_forward', dict(time=(1 << 31) - 1)),
     ('attention_forward', dict(time=4096, heads=1, workspace=0)),
     ('attention_forward', dict(time=4096, heads=1, workspace=4104)),
     *[('norm_forward', dict([(n, 0)])) for n in ('x', 'y')], ('norm_forward', dict(stats=4100)),
+    ('norm_forward', dict(width=(1 << 31) - 1)),
     *[('norm_backward', dict([(n, 0)])) for n in ('x', 'dy', 'stats', 'workspace')],
     ('norm_backward', dict(stats=4100)), ('norm_backward', dict(workspace=4104))])
 def test_launches_reject_what_is_not_there_or_not_aligned(name, args):
