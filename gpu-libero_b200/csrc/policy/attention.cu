@@ -235,11 +235,13 @@ Plan plan_of(const B200AttentionArgs *a, bool backward) {
   int widest = 0;
   for (int i = 0; i < p.scans; ++i) r.kt = std::max(r.kt, p.scan[i].kd), widest = std::max(widest, p.scan[i].vd);
   // Slices of v: 64 wide, or 32 where that is all there is; for wide heads also where
-  // slices of 64 would be half empty (300 rows of 200 tokens, 6 heads of 80 and 72 in
-  // bf16: 868 us with gradients against 948; of 96 and 104: 797 against 742), and for
-  // 32-bit ones, whose states of 64 columns leave one CTA an SM (696 us forward against
-  // 984; equal at 128).
-  const bool thin = r.kt > 64 && (a->dtype == B200_FP32 || widest <= 96);
+  // the last slice of 64 would be at most half full (300 rows of 200 tokens, 6 heads of
+  // 80 and 72 in bf16: 868 us with gradients against 948; of 96 and 104, whose last slice
+  // is fuller: 797 against 742; forward with one slice, 6 heads of 128 and 64: 172 us in
+  // two against 146, of 128 and 48: 183 against 163), and for 32-bit ones, whose states
+  // of 64 columns leave one CTA an SM (300 rows of 200, heads of 80 and 72: 696 us forward
+  // against 984; equal at 128).
+  const bool thin = r.kt > 64 && (a->dtype == B200_FP32 || (widest > 64 && widest <= 96));
   r.vt = widest <= 32 || thin ? 32 : 64;
   for (int i = 0; i < p.scans; ++i) {
     p.scan[i].vec_final = (uintptr_t)p.scan[i].final % 16 == 0;

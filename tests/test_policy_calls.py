@@ -151,3 +151,12 @@ def test_clip_rejects_missing_memory():
     for src, dst in ((0, 4096), (4096, 0)):
         with pytest.raises(RuntimeError, match='CUDA error 1$'):
             policy._lib().launch('clip', policy.native.PolicyLibrary.CLIP.pack(src, dst, 4, 0), 1, 1.0, 0.0, 256, 256, 0)
+
+
+def test_values_of_one_slice_are_not_cut_in_two():
+    """Wide keys with values of up to 64: one CTA a row and head, so that 80 of them are split over a long axis."""
+    shape = dict(time=500, heads=4, batch=20, dk=128)
+    for dtype in (1, 2):
+        assert attention_workspace(**shape, dv=64, dtype=dtype) and attention_workspace(**shape, dv=40, dtype=dtype)
+        for dv in (72, 96, 128):  # three slices of 32, or two of 64: more CTAs than SMs
+            assert not attention_workspace(**shape, dv=dv, dtype=dtype)
