@@ -14,7 +14,7 @@
 // fixed order.  Rows of more than 8192 are read again instead.
 // 262144 rows of 1024 in bf16: 184 us forward (5.8 TB/s) and 284 us backward (5.7
 // TB/s) and 8 us for the partial rows; 30011 rows of 771 floats, 1027 apart: 43 us
-// (4.3 TB/s) and 68 us (4.1 TB/s).
+// (4.3 TB/s) and 59 us (4.7 TB/s) with the partial rows.
 #include <algorithm>
 #include "common.cuh"
 
@@ -307,15 +307,29 @@ template <class T, int E, int R> struct Unit {
 // lane copies for itself, or, where rows start at any element, from the aligned
 // address before the row (the same allocation's memory) to the row's end.
 constexpr int kWarpThreads = 128;
-// CTAs of an SM, by their registers; the grid is one wave of them.
-__host__ __device__ constexpr int resident(int values, bool backward) {
+// Stages of the ring, and its bytes of a CTA, for rows of 32 `values` elements.
+__host__ __device__ constexpr int ring_stages(int values, int bytes, int tensors) { return values * bytes * tensors >= 128 ? 3 : 4; }
+__host__ __device__ constexpr int ring_row(int values, int bytes, bool single) { return 32 * values * bytes + (single ? 16 : 0); }
+__host__ __device__ constexpr int ring_bytes(int values, int bytes, bool single, int tensors) {
+  return ring_stages(values, bytes, tensors) * tensors * ring_row(values, bytes, single) * (kWarpThreads / 32);
+}
+// CTAs of an SM by their registers, and also by their shared memory (of 228 KB, 1 KB
+// more for each CTA; the backward pass also holds its sums); the grid is one wave of
+// them.  (32-bit rows of 513 to 1024, backward: two CTAs fit; a grid of three took 72 us
+// for 30011 rows of 771 instead of 59, and two stages that let three fit 64.)
+__host__ __device__ constexpr int by_registers(int values, bool backward) {
   return backward ? (values == 32 ? 3 : 4) : values == 32 ? 4 : values == 16 ? 5 : 8;
+}
+__host__ __device__ constexpr int resident(int values, bool backward, int bytes, bool single) {
+  const int held = ring_bytes(values, bytes, single, backward ? 2 : 1) + (backward ? 2 * 32 * values * 4 : 0) + 1024;
+  const int fit = 228 * 1024 / held, most = by_registers(values, backward);
+  return fit < most ? fit : most;
 }
 
 template <class T, int E, int R, int TENSORS> struct Ring {
-  static constexpr int kStages = R * sizeof(T) * TENSORS >= 128 ? 3 : 4;
-  static constexpr int kRow = 32 * R * sizeof(T) + (E == 1 ? 16 : 0);  // of one tensor and warp
-  static constexpr int bytes() { return kStages * TENSORS * kRow * (kWarpThreads / 32); }
+  static constexpr int kStages = ring_stages(R, sizeof(T), TENSORS);
+  static constexpr int kRow = ring_row(R, sizeof(T), E == 1);  // of one tensor and warp
+  static constexpr int bytes() { return ring_bytes(R, sizeof(T), E == 1, TENSORS); }
   static __device__ __forceinline__ int at(int stage, int tensor) {
     return ((stage * TENSORS + tensor) * (kWarpThreads / 32) + threadIdx.x / 32) * kRow;
   }
@@ -368,7 +382,7 @@ template <class T, int E, int R, int TENSORS> struct Ring {
 };
 
 template <class T, class W, int E, int R>
-__global__ void __launch_bounds__(kWarpThreads, resident(R, false)) forward_warps(B200NormArgs a) {
+__global__ void __launch_bounds__(kWarpThreads, resident(R, false, sizeof(T), E == 1)) forward_warps(B200NormArgs a) {
   using Rows = Ring<T, E, R, 1>;
   extern __shared__ __align__(16) unsigned char ring[];
   const int rank = threadIdx.x % 32, width = a.width;
@@ -454,7 +468,7 @@ __global__ void __launch_bounds__(kWarpThreads, resident(R, false)) forward_warp
 }
 
 template <class T, class W, int E, int R>
-__global__ void __launch_bounds__(kWarpThreads, resident(R, true)) backward_warps(B200NormArgs a, float *parts) {
+__global__ void __launch_bounds__(kWarpThreads, resident(R, true, sizeof(T), E == 1)) backward_warps(B200NormArgs a, float *parts) {
   using Rows = Ring<T, E, R, 2>;
   extern __shared__ __align__(16) unsigned char ring[];
   const int width = a.width;
@@ -659,7 +673,7 @@ Plan plan_of(const B200NormArgs *a, bool backward) {
   // Enough CTAs to fill the SMs; in the backward pass no more than are resident
   // at once, as each leaves a partial row.
   const int groups = p.group == 32 ? kWarpThreads / 32 : p.group ? threads_of(p.group) / p.group : 1;
-  const int most = p.group == 32 ? resident(p.values, backward)
+  const int most = p.group == 32 ? resident(p.values, backward, (int)bytes, !blocks)
                    : !backward   ? 16
                    : p.group == 128 ? 6 : p.group == 512 ? 2 : 3;
   // a handful of rows: one CTA's sums are the totals, which saves a launch

@@ -160,3 +160,12 @@ def test_values_of_one_slice_are_not_cut_in_two():
         assert attention_workspace(**shape, dv=64, dtype=dtype) and attention_workspace(**shape, dv=40, dtype=dtype)
         for dv in (72, 96, 128):  # three slices of 32, or two of 64: more CTAs than SMs
             assert not attention_workspace(**shape, dv=dv, dtype=dtype)
+
+
+@pytest.mark.parametrize('width,row,dtype,ctas', [
+    (771, 1027, 0, 2), (1024, 1024, 0, 2), (513, 513, 0, 2), (512, 512, 0, 4), (256, 256, 0, 4),
+    (1024, 1024, 1, 3), (771, 771, 2, 3), (512, 512, 2, 4), (256, 256, 1, 4)])
+def test_norm_gradients_take_one_wave_of_ctas(width, row, dtype, ctas):
+    """A partial row for each CTA: as many as an SM's shared memory holds (228 KB, 1 KB more for each CTA)."""
+    args = norm_args(rows=30011, width=width, x_row=row, dy_row=width, dtype=dtype, workspace=0)
+    assert policy._lib().size('norm', args) == 148 * ctas * 2 * width * 4
