@@ -235,12 +235,12 @@ Plan plan_of(const B200AttentionArgs *a, bool backward) {
   int widest = 0;
   for (int i = 0; i < p.scans; ++i) r.kt = std::max(r.kt, p.scan[i].kd), widest = std::max(widest, p.scan[i].vd);
   // Slices of v: 64 wide, or 32 where that is all there is; for wide heads also where
-  // the last slice of 64 would be at most half full (300 rows of 200 tokens, 6 heads of
-  // 80 and 72 in bf16: 868 us with gradients against 948; of 96 and 104, whose last slice
-  // is fuller: 797 against 742; forward with one slice, 6 heads of 128 and 64: 172 us in
-  // two against 146, of 128 and 48: 183 against 163), and for 32-bit ones, whose states
-  // of 64 columns leave one CTA an SM (300 rows of 200, heads of 80 and 72: 696 us forward
-  // against 984; equal at 128).
+  // the last slice of 64 would be at most half full (300 rows of 200 tokens and 6 heads
+  // in bf16: of 80 and 72, 936 us with gradients against 1010; 200 such rows of 96 and
+  // 104, whose last slice is fuller, 782 against 720; forward with one slice, of 128 and
+  // 64, 173 us in two against 146, of 128 and 48, 183 against 163), and for 32-bit ones,
+  // whose states of 64 columns leave one CTA an SM (of 80 and 72, 746 us forward against
+  // 1052; of 128, 1220 against 1256).
   const bool thin = r.kt > 64 && (a->dtype == B200_FP32 || (widest > 64 && widest <= 96));
   r.vt = widest <= 32 || thin ? 32 : 64;
   for (int i = 0; i < p.scans; ++i) {
@@ -266,7 +266,10 @@ Plan plan_of(const B200AttentionArgs *a, bool backward) {
   // Rows are split where they are fewer than the SMs, into as many pieces as are
   // resident at once, of two chunks at least.  A piece reads its keys and values
   // twice, about 1.4 times the work, and takes two launches more (256 rows of 256
-  // tokens and 64 wide: 93 us in two pieces each).
+  // tokens and 64 wide: 27 us whole, 93 in two pieces each).  From there on rows stay
+  // whole however long they are: of 4000 tokens, 147 rows of 64 wide take 168 us in
+  // pieces and 148 take 201; on tcgen05, with one CTA an SM, 74 rows of two slices take
+  // 156 and 75 take 297, for a second wave of two CTAs.
   const int64_t rows = (int64_t)p.batch * p.heads * p.units;
   const int tile = r.tc ? kTcTile : kTile, chunks = (p.time + tile - 1) / tile;
   const int resident = r.tc ? 1

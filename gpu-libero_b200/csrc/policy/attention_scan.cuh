@@ -20,7 +20,7 @@
 // one piece of the row, and walks the chunks; the next chunk's loads fly meanwhile.
 //
 // What bounds it: not one unit alone.  For 1184 rows of 256 tokens and 4 heads of 64
-// in bf16 (214 us forward, 56% of the copy bandwidth; 746 us with the gradients) the
+// in bf16 (215 us forward, 56% of the copy bandwidth; 750 us with the gradients) the
 // tensor pipe is busy 39% of the time, the instruction slots half of it and shared
 // memory's pipe 60%, with 16 warps an SM; what is left are the warps' waits for each
 // other's and their own results.  The main loop has to fit the instruction cache:

@@ -12,9 +12,9 @@
 // the same columns in every row, so that the sums over rows of dweight and dbias stay
 // in its registers; CTAs leave one partial row each, which a second kernel adds in a
 // fixed order.  Rows of more than 8192 are read again instead.
-// 262144 rows of 1024 in bf16: 184 us forward (5.8 TB/s) and 284 us backward (5.7
-// TB/s) and 8 us for the partial rows; 30011 rows of 771 floats, 1027 apart: 43 us
-// (4.3 TB/s) and 59 us (4.7 TB/s) with the partial rows.
+// 262144 rows of 1024 in bf16: 200 us forward (5.4 TB/s) and 279 us backward (5.8
+// TB/s), 8 of them for the partial rows; 30011 rows of 771 floats, 1027 apart: 43 us
+// (4.3 TB/s) and 59 us (4.7 TB/s).
 #include <algorithm>
 #include "common.cuh"
 
